@@ -228,6 +228,25 @@ def _stream(stream=None):
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()) or STREAM_LEGACY
 
 
+def _torch_stream(stream, device):
+    """The torch stream of `stream` (a torch stream or a raw handle of a stream of `device`)."""
+    if getattr(stream, "cuda_stream", None) is not None:
+        return stream
+    if stream in (0, STREAM_LEGACY):
+        return torch.cuda.default_stream(device)
+    return torch.cuda.ExternalStream(stream, device)
+
+
+def _new(shape, dtype, device, stream=None, make=torch.empty):
+    """A call's new tensor, made (and cleared, with make=torch.zeros) on the stream that the call runs on: a tensor belongs
+    to the stream that is current when it is made, whose earlier work may still use its memory and whose later tensors get
+    that memory once it is dropped."""
+    if stream is None:
+        return make(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(_torch_stream(stream, device)):
+        return make(shape, dtype=dtype, device=device)
+
+
 def _host_stream(stream=None):
     """As _stream for calls that read or write host buffers: torch's default stream is NULL here, so that the call has
     finished with those buffers when it returns."""
@@ -260,28 +279,28 @@ def quantize_rows(t, x, out=None, stream=None):
     """Float rows (device fp32, a whole number of blocks) -> `t` blocks (uint8 device tensor)."""
     n = x.numel()
     if out is None:
-        out = torch.empty(n // BLOCK_VALUES[t] * BLOCK_BYTES[t], dtype=torch.uint8, device=x.device)
+        out = _new(n // BLOCK_VALUES[t] * BLOCK_BYTES[t], torch.uint8, x.device, stream)
     _check(lib().xs_quantize_rows(t, _p(x), n, _p(out), _stream(stream)))
     return out
 
 
 def iq_dequant_f32(t, src, n, out=None, stream=None):
     if out is None:
-        out = torch.empty(n, dtype=torch.float32, device=src.device)
+        out = _new(n, torch.float32, src.device, stream)
     _check(lib().xs_iq_dequant_f32(t, _p(src), n, _p(out), _stream(stream)))
     return out
 
 
 def iq_dequant_bf16(t, src, n, out=None, stream=None):
     if out is None:
-        out = torch.empty(n, dtype=torch.int16, device=src.device)
+        out = _new(n, torch.int16, src.device, stream)
     _check(lib().xs_iq_dequant_bf16(t, _p(src), n, _p(out), _stream(stream)))
     return out
 
 
 def iq_dequant_f16(t, src, n, out=None, stream=None):
     if out is None:
-        out = torch.empty(n, dtype=torch.float16, device=src.device)
+        out = _new(n, torch.float16, src.device, stream)
     _check(lib().xs_iq_dequant_f16(t, _p(src), n, _p(out), _stream(stream)))
     return out
 
@@ -292,7 +311,7 @@ def quantize_q8_1_rows(x, out=None, stream=None):
     """x [rows, cols] fp32 -> q8_1 blocks, rows * cols / 32 * 36 bytes (reference quantize_q8_1_rows)."""
     rows, cols = x.shape
     if out is None:
-        out = torch.empty(rows * cols // 32 * 36, dtype=torch.uint8, device=x.device)
+        out = _new(rows * cols // 32 * 36, torch.uint8, x.device, stream)
     _check(lib().xs_quantize_q8_1_rows(_p(x), rows, cols, _p(out), _stream(stream)))
     return out
 
@@ -303,17 +322,17 @@ def router_top10(logits, k, ids=None, weights=None, stream=None):
     """logits [T, E] fp32 -> (ids [T, k] int32, weights [T, k] fp32) (reference router_top10)."""
     T, E = logits.shape
     if ids is None:
-        ids = torch.empty(T, k, dtype=torch.int32, device=logits.device)
+        ids = _new((T, k), torch.int32, logits.device, stream)
     if weights is None:
-        weights = torch.empty(T, k, dtype=torch.float32, device=logits.device)
+        weights = _new((T, k), torch.float32, logits.device, stream)
     _check(lib().xs_router_top10(_p(logits), T, E, k, _p(ids), _p(weights), _stream(stream)))
     return ids, weights
 
 
 def router_grouped_sigmoid(logits, bias, n_group, topk_group, k, routed_scale, stream=None):
     T, E = logits.shape
-    ids = torch.empty(T, k, dtype=torch.int32, device=logits.device)
-    weights = torch.empty(T, k, dtype=torch.float32, device=logits.device)
+    ids = _new((T, k), torch.int32, logits.device, stream)
+    weights = _new((T, k), torch.float32, logits.device, stream)
     _check(lib().xs_router_grouped_sigmoid(_p(logits), _p(bias), T, E, n_group, topk_group, k, float(routed_scale),
                                            _p(ids), _p(weights), _stream(stream)))
     return ids, weights
@@ -322,7 +341,7 @@ def router_grouped_sigmoid(logits, bias, n_group, topk_group, k, routed_scale, s
 def router_logits_f32(x, w, stream=None):
     T, H = x.shape
     E = w.shape[0]
-    logits = torch.empty(T, E, dtype=torch.float32, device=x.device)
+    logits = _new((T, E), torch.float32, x.device, stream)
     _check(lib().xs_router_logits_f32(_p(x), _p(w), _p(logits), T, H, E, _stream(stream)))
     return logits
 
@@ -348,12 +367,12 @@ def prefill_route(ids, k, n_expert, cache_base=None, blob=0, with_ptr=False, str
     """ids [T*k] -> dict(src, slot, entry, bounds, experts, n_groups, grp_ptr) (reference plain_prompt.cpp:576-637)."""
     n = ids.numel()
     dev = ids.device
-    o = dict(src=torch.empty(n, dtype=torch.int32, device=dev), slot=torch.empty(n, dtype=torch.int32, device=dev),
-             entry=torch.empty(n, dtype=torch.int32, device=dev),
-             bounds=torch.empty(n_expert + 1, dtype=torch.int32, device=dev),
-             experts=torch.empty(n_expert, dtype=torch.int32, device=dev),
-             n_groups=torch.empty(1, dtype=torch.int32, device=dev),
-             grp_ptr=torch.empty(n_expert, dtype=torch.int64, device=dev) if with_ptr else None)
+    o = dict(src=_new(n, torch.int32, dev, stream), slot=_new(n, torch.int32, dev, stream),
+             entry=_new(n, torch.int32, dev, stream),
+             bounds=_new(n_expert + 1, torch.int32, dev, stream),
+             experts=_new(n_expert, torch.int32, dev, stream),
+             n_groups=_new(1, torch.int32, dev, stream),
+             grp_ptr=_new(n_expert, torch.int64, dev, stream) if with_ptr else None)
     _check(lib().xs_prefill_route(_p(ids), n, k, n_expert, _p(o["src"]), _p(o["slot"]), _p(o["entry"]),
                                   _p(o["bounds"]), _p(o["experts"]), _p(o["n_groups"]), cache_base, blob,
                                   _p(o["grp_ptr"]), _stream(stream)))
@@ -403,7 +422,7 @@ def f32_gemv_fp32_mmvf_multi(x, w, n_tok=None, out=None, stream=None):
     n_tok = x.shape[0] if n_tok is None else n_tok
     n_out, n_in = w.shape
     if out is None:
-        out = torch.empty(n_tok, n_out, dtype=torch.float32, device=x.device)
+        out = _new((n_tok, n_out), torch.float32, x.device, stream)
     fn = lib().xs_bf16_gemv_fp32_mmvf_multi if w.dtype in (torch.int16, torch.bfloat16) else \
         lib().xs_f32_gemv_fp32_mmvf_multi
     _check(fn(_p(x), x.stride(0), _p(w), _p(out), out.stride(0), n_in, n_out, n_tok, _stream(stream)))
@@ -415,7 +434,7 @@ def f32_gemm_rows(x, w, out=None, stream=None):
     n_tok, n_in = x.shape
     n_out = w.shape[0]
     if out is None:
-        out = torch.empty(n_tok, n_out, dtype=torch.float32, device=x.device)
+        out = _new((n_tok, n_out), torch.float32, x.device, stream)
     _check(lib().xs_f32_gemm_rows(_p(x), x.stride(0), _p(w), _p(out), out.stride(0), n_in, n_out, n_tok,
                                   _stream(stream)))
     return out
@@ -423,7 +442,7 @@ def f32_gemm_rows(x, w, out=None, stream=None):
 
 def f32_to_bf16_bulk(x, out=None, stream=None):
     if out is None:
-        out = torch.empty(x.numel(), dtype=torch.int16, device=x.device)
+        out = _new(x.numel(), torch.int16, x.device, stream)
     _check(lib().xs_f32_to_bf16_bulk(_p(x), _p(out), x.numel(), _stream(stream)))
     return out
 
@@ -432,7 +451,7 @@ def bf16_gemv(x, w, out=None, threads_per_row=None, stream=None):
     """x bf16 bits [n_in], w bf16 bits [n_out, n_in]: bf16_gemv, or bf16_gemv_split at threads_per_row."""
     n_out, n_in = w.shape
     if out is None:
-        out = torch.empty(n_out, dtype=torch.float32, device=w.device)
+        out = _new(n_out, torch.float32, w.device, stream)
     if threads_per_row is None:
         _check(lib().xs_bf16_gemv(_p(x), _p(w), _p(out), n_in, n_out, _stream(stream)))
     else:
@@ -443,7 +462,7 @@ def bf16_gemv(x, w, out=None, threads_per_row=None, stream=None):
 def project_bf16(x, w, split=True, native=False, x_bf16=None, out=None, stream=None):
     n_out, n_in = w.shape
     if out is None:
-        out = torch.empty(n_out, dtype=torch.float32, device=w.device)
+        out = _new(n_out, torch.float32, w.device, stream)
     _check(lib().xs_project_bf16(_p(x), _p(x_bf16), _p(w), _p(out), n_in, n_out, int(split), int(native),
                                  _stream(stream)))
     return out
@@ -466,7 +485,7 @@ def iq_mmq_type_dup(t):
 def iq_mmq_quantize(x, ids, cols, ld, rows, sums, dup=False, out=None, stream=None):
     """int8 MMQ activations (xs_iq_mmq_quantize): a uint8 device tensor of iq_mmq_act_bytes(rows, oc) bytes."""
     if out is None:
-        out = torch.zeros(iq_mmq_act_bytes(rows, 2 * cols if dup else cols), dtype=torch.uint8, device=x.device)
+        out = _new(iq_mmq_act_bytes(rows, 2 * cols if dup else cols), torch.uint8, x.device, stream, torch.zeros)
     _check(lib().xs_iq_mmq_quantize(_p(x), _p(ids), _p(out), cols, ld, rows, int(sums), int(dup), _stream(stream)))
     return out
 
@@ -484,8 +503,7 @@ def iq_mmq_grouped(type_, w, expert_bytes, w_rows, w_cols, n, xq, total_rows, bo
 
 def iq_mmq_quantize_scatter(x, slot, cols, ld, tokens, k_used, sums, dup=False, out=None, stream=None):
     if out is None:
-        out = torch.zeros(iq_mmq_act_bytes(tokens * k_used, 2 * cols if dup else cols), dtype=torch.uint8,
-                          device=x.device)
+        out = _new(iq_mmq_act_bytes(tokens * k_used, 2 * cols if dup else cols), torch.uint8, x.device, stream, torch.zeros)
     _check(lib().xs_iq_mmq_quantize_scatter(_p(x), _p(slot), _p(out), cols, ld, tokens, k_used, int(sums), int(dup),
                                             _stream(stream)))
     return out
@@ -493,14 +511,14 @@ def iq_mmq_quantize_scatter(x, slot, cols, ld, tokens, k_used, sums, dup=False, 
 
 def mmq_swiglu(gu, rows, n_ff, interleaved, out=None, stream=None):
     if out is None:
-        out = torch.empty(rows, n_ff, dtype=torch.float32, device=gu.device)
+        out = _new((rows, n_ff), torch.float32, gu.device, stream)
     _check(lib().xs_mmq_swiglu(_p(gu), _p(out), rows, n_ff, int(interleaved), _stream(stream)))
     return out
 
 
 def mmq_iota(n, out=None, device="cuda", stream=None):
     if out is None:
-        out = torch.empty(n, dtype=torch.int32, device=device)
+        out = _new(n, torch.int32, device, stream)
     _check(lib().xs_mmq_iota(_p(out), n, _stream(stream)))
     return out
 
@@ -550,9 +568,9 @@ def shared_expert_decode(SL, blob, x, w_gate=None, stream=None):
     rows [T, n_embd], gate logits [T] or None)."""
     T = x.shape[0]
     ws_bytes = lib().xs_shared_expert_decode_workspace_bytes(ctypes.byref(SL), T)
-    ws = torch.zeros(ws_bytes + 256, dtype=torch.uint8, device=x.device)
-    shared = torch.empty(T, SL.n_embd, dtype=torch.float32, device=x.device)
-    gate = torch.empty(T, dtype=torch.float32, device=x.device) if w_gate is not None else None
+    ws = _new(ws_bytes + 256, torch.uint8, x.device, stream, torch.zeros)
+    shared = _new((T, SL.n_embd), torch.float32, x.device, stream)
+    gate = _new(T, torch.float32, x.device, stream) if w_gate is not None else None
     _check(lib().xs_shared_expert_decode(ctypes.byref(SL), _p(blob), _p(x), T, _p(w_gate), _p(shared), _p(gate),
                                          (ws.data_ptr() + 255) & ~255, ws_bytes, _stream(stream)))
     return shared, gate
@@ -697,7 +715,7 @@ def _codes(what, name, q, scale, dev=None, n=None):
     return rows, n, ld, at
 
 
-def _float_out(what, name, out, out_type, rows, n, x):
+def _float_out(what, name, out, out_type, rows, n, x, stream):
     """A call's rows of floats: those given, or new ones of out_type (None: none) -> (out, its row stride, its type's id)."""
     if out is not None:
         return (out, *_rows(what, name, out, x.get_device(), rows, n)[2:])
@@ -706,10 +724,10 @@ def _float_out(what, name, out, out_type, rows, n, x):
     code = FLOAT_TYPE.get(out_type)
     if code is None:
         raise _bad(f"{what}: {name} is {out_type}")
-    return x.new_empty((rows, n), dtype=out_type), n, code
+    return x.new_empty((rows, n), dtype=out_type) if stream is None else _new((rows, n), out_type, x.device, stream), n, code
 
 
-def _int8_out(what, quant, q, scale, rows, n, x):
+def _int8_out(what, quant, q, scale, rows, n, x, stream):
     """A call's int8 rows: those given, or new ones with quant -> (q, scale, q's address, its row stride, scale's address)."""
     if q is None:
         if not quant:
@@ -717,7 +735,7 @@ def _int8_out(what, quant, q, scale, rows, n, x):
                 raise _bad(f"{what}: scales without codes")
             return None, None, None, 0, None
         ld = (n + 15) & ~15
-        q = x.new_empty((rows, ld), dtype=torch.int8)
+        q = x.new_empty((rows, ld), dtype=torch.int8) if stream is None else _new((rows, ld), torch.int8, x.device, stream)
         at = q.data_ptr()
         if ld != n:
             q = q[:, :n]
@@ -725,13 +743,15 @@ def _int8_out(what, quant, q, scale, rows, n, x):
         ld = _rows(what, "q", q, x.get_device(), rows, n, INT8_TYPE)[2]
         at = q.data_ptr()
     if scale is None:
-        scale = x.new_empty((rows,), dtype=torch.float32)
+        scale = x.new_empty((rows,), dtype=torch.float32) if stream is None else _new((rows,), torch.float32, x.device, stream)
         return q, scale, at, ld, scale.data_ptr()
     return q, scale, at, ld, _vec(what, "scale", scale, rows, x.get_device())
 
 
 def _launch(fn, dev, stream, args):
     """The entry point `fn` on `dev` (made the current device where it is not) and its current stream, or `stream`."""
+    if stream is not None and getattr(stream, "device_index", dev) != dev:
+        raise _bad(f"a stream of cuda:{stream.device_index} for tensors on cuda:{dev}")
     if torch._C._cuda_getDevice() != dev:
         with torch.cuda.device(dev):
             _check(fn(*args, _stream(stream)))
@@ -747,8 +767,8 @@ def block_norm(x, w=None, eps=1e-6, out_type=torch.float32, quant=False, out=Non
     what = "block_norm"
     T, n, ldx, xt = _rows(what, "x", x)
     dev = x.get_device()
-    out, ldy, yt = _float_out(what, "out", out, out_type, T, n, x)
-    q, scale, qp, ldq, sp = _int8_out(what, quant, q, scale, T, n, x)
+    out, ldy, yt = _float_out(what, "out", out, out_type, T, n, x, stream)
+    q, scale, qp, ldq, sp = _int8_out(what, quant, q, scale, T, n, x, stream)
     _launch(lib().xs_block_norm, dev, stream,
             (x.data_ptr(), xt, ldx, _vec(what, "w", w, n, dev), eps, _p(out), yt, ldy, qp, ldq, sp, T, n))
     return out, q, scale
@@ -807,13 +827,16 @@ def _join(what, fn, head, x, residual, cfg, T, n, out, next_type, next, quant, q
             _vec(what, "gate", gate, T if cfg.gate_kind == 1 else n, dev)
     _, _, ldr, rt = _rows(what, "residual", residual, dev, T, n)
     if out is None:
-        out = residual.new_empty((T, n)) if ldr == n else             torch.empty_strided((T, n), (ldr, 1), dtype=residual.dtype, device=residual.device)
+        if ldr == n:
+            out = residual.new_empty((T, n)) if stream is None else _new((T, n), residual.dtype, residual.device, stream)
+        else:
+            out = _new(max(T - 1, 0) * ldr + n, residual.dtype, residual.device, stream).as_strided((T, n), (ldr, 1))
     elif out is not residual:
         ldo = _rows(what, "out", out, dev, T, n, {residual.dtype: rt})[2]
         if ldo != ldr and T > 1:
             raise _bad(f"{what}: out's rows are {ldo} values apart, the residual's {ldr}")
-    next, ldn, nt = _float_out(what, "next", next, next_type, T, n, x)
-    q, scale, qp, ldq, sp = _int8_out(what, quant, q, scale, T, n, x)
+    next, ldn, nt = _float_out(what, "next", next, next_type, T, n, x, stream)
+    q, scale, qp, ldq, sp = _int8_out(what, quant, q, scale, T, n, x, stream)
     _launch(fn, dev, stream, (ctypes.addressof(cfg), *head, residual.data_ptr(), out.data_ptr(), rt, ldr, _p(next), nt, ldn,
                               qp, ldq, sp, T, n))
     return out, next, q, scale
@@ -849,7 +872,7 @@ def w8a8_quantize(x, q=None, scale=None, stream=None):
     """Rows x [rows, n] -> int8 rows (q [rows, n], scale [rows]): activations, or a weight matrix's outputs."""
     what = "w8a8_quantize"
     rows, n, ldx, xt = _rows(what, "x", x)
-    q, scale, qp, ldq, sp = _int8_out(what, True, q, scale, rows, n, x)
+    q, scale, qp, ldq, sp = _int8_out(what, True, q, scale, rows, n, x, stream)
     _launch(lib().xs_w8a8_quantize, x.get_device(), stream, (x.data_ptr(), xt, ldx, qp, ldq, sp, rows, n))
     return q, scale
 
@@ -862,7 +885,7 @@ def w8a8_gemm(q, scale, w, w_scale, out_type=torch.float32, out=None, stream=Non
     n_out, _, ldw, ws = _codes(what, "w", w, w_scale, dev, n_in)
     if out is None and out_type is None:
         raise _bad(f"{what}: no output")
-    out, ldy, yt = _float_out(what, "out", out, out_type, T, n_out, q)
+    out, ldy, yt = _float_out(what, "out", out, out_type, T, n_out, q, stream)
     _launch(lib().xs_w8a8_gemm, dev, stream,
             (q.data_ptr(), ldx, xs, w.data_ptr(), ldw, ws, out.data_ptr(), yt, ldy, T, n_in, n_out))
     return out
@@ -879,7 +902,7 @@ def w8a8_swiglu(q, scale, w_gate, gate_scale, w_up, up_scale, out_type=torch.flo
         raise _bad(f"{what}: the up rows are not laid out as the gate rows ({n_up} at {ldu} bytes, {n_ff} at {ldw})")
     if out is None and out_type is None:
         raise _bad(f"{what}: no output")
-    out, ldh, ht = _float_out(what, "out", out, out_type, T, n_ff, q)
+    out, ldh, ht = _float_out(what, "out", out, out_type, T, n_ff, q, stream)
     _launch(lib().xs_w8a8_swiglu, dev, stream,
             (q.data_ptr(), ldx, xs, w_gate.data_ptr(), gs, w_up.data_ptr(), us, ldw, out.data_ptr(), ht, ldh, T, n_in, n_ff))
     return out
