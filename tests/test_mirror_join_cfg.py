@@ -1,0 +1,86 @@
+"""A join's configuration whose tensors are given other memory, sizes or types after it was made: the calls take them as they
+then are, or refuse them (no GPU: the library is stood in for, and shows the configuration that it was handed)."""
+import ctypes
+
+import pytest
+import torch
+from torch.overrides import TorchFunctionMode
+
+import xsmoe
+
+
+class OnDevice(TorchFunctionMode):
+    def __torch_function__(self, func, types, args=(), kwargs=None):
+        if getattr(func, "__name__", "") == "get_device":
+            return 0
+        return func(*args, **(kwargs or {}))
+
+
+@pytest.fixture
+def handed(monkeypatch):
+    """The configuration that the last call handed to the library: [norm_w, gate, ld_gate, next_w, scales ...]."""
+    got = []
+
+    class Lib:
+        def xs_block_join(self, j, *a):
+            c = xsmoe.BlockJoinCfg.from_address(j)
+            got[:] = [getattr(c, n) for n, _ in c._fields_]
+            return 0
+
+    monkeypatch.setattr(xsmoe, "lib", lambda: Lib())
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 0, raising=False)
+    with OnDevice():
+        yield got
+
+
+T, N = 3, 64
+
+
+def case(gate_kind="token"):
+    gate = {"token": torch.ones(T), "channel": torch.ones(N), "value": torch.ones(T, 2 * N)[:, :N]}[gate_kind]
+    v = dict(norm=True, norm_w=torch.ones(N), norm_eps=1e-5, gate=gate, gate_kind=gate_kind, branch_scale=0.5,
+             residual_scale=0.25, next_w=torch.ones(N), next_eps=1e-4)
+    return v, xsmoe.block_join_cfg(**v)
+
+
+def join(cfg):
+    return xsmoe.block_join(torch.ones(T, N), torch.ones(T, N), cfg, quant=True)
+
+
+def fields(v):
+    c = xsmoe.block_join_cfg(**v)
+    return [getattr(c, n) for n, _ in c._fields_]
+
+
+@pytest.mark.parametrize("which", ["norm_w", "gate", "next_w"])
+@pytest.mark.parametrize("gate_kind", ["token", "channel", "value"])
+def test_other_memory_is_taken(handed, gate_kind, which):
+    v, cfg = case(gate_kind)
+    join(cfg)
+    assert handed == fields(v)
+    was = list(handed)
+    t, old = v[which], v[which].data      # (the old memory is kept: an address of it would be told)
+    t.data = torch.full(t.shape, 2.0)     # the value gate's rows closer together, too
+    join(cfg)
+    assert handed == fields(v) and handed != was
+    t.data = old
+    join(cfg)
+    assert handed == was
+
+
+@pytest.mark.parametrize("which", ["norm_w", "gate", "next_w"])
+@pytest.mark.parametrize("gate_kind", ["token", "channel", "value"])
+def test_what_no_longer_fits_is_refused(handed, gate_kind, which):
+    for spoil in (lambda t: torch.ones([n - 1 for n in t.shape]), lambda t: torch.ones(t.shape, dtype=torch.float16),
+                  lambda t: torch.ones([2 * n for n in t.shape])[tuple(slice(None, None, 2) for _ in t.shape)]):
+        v, cfg = case(gate_kind)
+        v[which].data = spoil(v[which])
+        with pytest.raises(xsmoe.XsError, match=which):
+            join(cfg)
+    if gate_kind == "value" and which == "gate":
+        return
+    v, cfg = case(gate_kind)
+    v[which].resize_(v[which].numel() - 1)                # the same address
+    with pytest.raises(xsmoe.XsError, match=which):
+        join(cfg)

@@ -652,6 +652,7 @@ class MoeLayer:
 FLOAT_TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 INT8_TYPE = {torch.int8: 24}
 GATE_KIND = {"none": 0, "token": 1, "channel": 2, "value": 3}
+_GATE_NAME = list(GATE_KIND)
 
 
 def _bad(message):
@@ -777,7 +778,8 @@ def block_norm(x, w=None, eps=1e-6, out_type=torch.float32, quant=False, out=Non
 def block_join_cfg(norm=False, norm_w=None, norm_eps=1e-6, gate=None, gate_kind="none", branch_scale=1.0,
                    residual_scale=1.0, next_w=None, next_eps=1e-6):
     """How a block's output joins the residual stream (include/xs_block.h): a BlockJoinCfg with its tensors kept alive.
-    gate_kind: none, token (gate [T], through a sigmoid), channel (gate [n]) or value (gate [T, n])."""
+    gate_kind: none, token (gate [T], through a sigmoid), channel (gate [n]) or value (gate [T, n]).  Calls take the tensors
+    as they then are, whatever memory they have been given since."""
     what = "block_join_cfg"
     if gate_kind not in GATE_KIND:
         raise _bad(f"{what}: gate kind {gate_kind!r}")
@@ -805,6 +807,18 @@ def block_join_cfg(norm=False, norm_w=None, norm_eps=1e-6, gate=None, gate_kind=
             T = many if size is None else t.shape[0]
         plain = plain and t.dtype is torch.float32 and (size == -3 or t.is_contiguous())
     cfg._for, cfg._plain = (T, n, dev), plain
+    cfg._seen = [(t, t.data_ptr(), t.dtype, t.shape, t.stride()) for t in cfg._keep if t is not None]
+    return cfg
+
+
+def _as_it_is(cfg):
+    """The configuration, made again (for this call) where one of its tensors has since been given other memory, another size,
+    layout or type."""
+    for t, at, kind, shape, stride in cfg._seen:
+        if t.data_ptr() != at or t.dtype is not kind or t.shape != shape or t.stride() != stride:
+            norm_w, gate, next_w = cfg._keep
+            return block_join_cfg(cfg.norm == 1, norm_w, cfg.norm_eps, gate, _GATE_NAME[cfg.gate_kind], cfg.branch_scale,
+                                  cfg.residual_scale, next_w, cfg.next_eps)
     return cfg
 
 
@@ -816,6 +830,7 @@ _GATE_FOR = {"none": (None, None), "token": (True, None), "channel": (None, -2),
 def _join(what, fn, head, x, residual, cfg, T, n, out, next_type, next, quant, q, scale, stream):
     """What block_join and moe_combine_join share: the configuration's and the outputs' checks, then the call."""
     dev = x.get_device()
+    cfg = _as_it_is(cfg)
     rows, size, at = cfg._for
     if not (cfg._plain and (rows is None or rows == T) and (size is None or size == n) and (at is None or at == dev)):
         norm_w, gate, next_w = cfg._keep   # one of them does not fit: say which
