@@ -27,6 +27,9 @@ def handed(monkeypatch):
             got[:] = [getattr(c, n) for n, _ in c._fields_]
             return 0
 
+        def xs_block_norm(self, *a):
+            return 0
+
     monkeypatch.setattr(xsmoe, "lib", lambda: Lib())
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 0, raising=False)
@@ -84,3 +87,21 @@ def test_what_no_longer_fits_is_refused(handed, gate_kind, which):
     v[which].resize_(v[which].numel() - 1)                # the same address
     with pytest.raises(xsmoe.XsError, match=which):
         join(cfg)
+    v, cfg = case(gate_kind)
+    v[which].untyped_storage().resize_(0)                 # an address of NULL would mean no weights
+    assert "freed" in message(lambda: join(cfg))
+
+
+def message(call):
+    """What the call raises, in words (a failing test's report would read its freed tensors)."""
+    try:
+        call()
+    except Exception as e:
+        return str(e)
+    return "nothing"
+
+
+def test_freed_weights_are_refused(handed):
+    w = torch.ones(N)
+    w.untyped_storage().resize_(0)
+    assert "w's memory has been freed" in message(lambda: xsmoe.block_norm(torch.ones(T, N), w))

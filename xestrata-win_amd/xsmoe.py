@@ -692,7 +692,10 @@ def _vec(what, name, t, n, dev):
         return None
     if isinstance(t, torch.Tensor) and t.get_device() == dev and t.dtype is torch.float32 and t.numel() == n and \
             t.is_contiguous():
-        return t.data_ptr()
+        at = t.data_ptr()
+        if at or not n:
+            return at
+        raise _bad(f"{what}: {name}'s memory has been freed")   # (0 would be NULL: no weights, no gate)
     if not isinstance(t, torch.Tensor) or t.get_device() != dev:
         raise _bad(f"{what}: {name} is not a tensor on cuda:{dev}")
     raise _bad(f"{what}: {name} is not {n} fp32 values in a row")
@@ -805,7 +808,7 @@ def block_join_cfg(norm=False, norm_w=None, norm_eps=1e-6, gate=None, gate_kind=
             n = t.shape[1] if n is None or n == t.shape[1] else -1
         if rows is not None:
             T = many if size is None else t.shape[0]
-        plain = plain and t.dtype is torch.float32 and (size == -3 or t.is_contiguous())
+        plain = plain and t.dtype is torch.float32 and (size == -3 or t.is_contiguous()) and (t.data_ptr() != 0 or many == 0)
     cfg._for, cfg._plain = (T, n, dev), plain
     cfg._seen = [(t, t.data_ptr(), t.dtype, t.shape, t.stride()) for t in cfg._keep if t is not None]
     return cfg
