@@ -30,6 +30,10 @@ def handed(monkeypatch):
         def xs_block_norm(self, *a):
             return 0
 
+        def xs_moe_combine_join(self, j, parts, weights, k, *a):
+            got[:] = [weights, k]
+            return 0
+
     monkeypatch.setattr(xsmoe, "lib", lambda: Lib())
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
     monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 0, raising=False)
@@ -105,3 +109,14 @@ def test_freed_weights_are_refused(handed):
     w = torch.ones(N)
     w.untyped_storage().resize_(0)
     assert "w's memory has been freed" in message(lambda: xsmoe.block_norm(torch.ones(T, N), w))
+
+
+def test_one_row_of_a_wider_buffers_weights(handed):
+    """The stride of one row says nothing; that of two has to be k."""
+    buffer, cfg = torch.ones(4, 6), xsmoe.block_join_cfg()
+    for row in (0, 3):
+        w = buffer[row:row + 1, 2:5]
+        xsmoe.moe_combine_join(torch.ones(3, N), w, torch.ones(1, N), cfg)
+        assert handed == [w.data_ptr(), 3]
+    with pytest.raises(xsmoe.XsError, match="6 values apart"):
+        xsmoe.moe_combine_join(torch.ones(6, N), buffer[:2, :3], torch.ones(2, N), cfg)

@@ -878,7 +878,7 @@ def moe_combine_join(parts, weights, residual, cfg, shared=None, shared_gate=Non
     n = _rows(what, "residual", residual, dev, T)[1]
     if parts is None:
         raise _bad(f"{what}: no parts")
-    if ldw != k:
+    if ldw != k and T > 1:
         raise _bad(f"{what}: the weights' rows are {ldw} values apart, not {k}")
     head = (_vec(what, "parts", parts, T * k * n, dev), weights.data_ptr(), k, _vec(what, "shared", shared, T * n, dev),
             _vec(what, "shared_gate", shared_gate, T, dev))
