@@ -5,9 +5,11 @@
 //          out = fl(fl(rs residual) + fl(bs b)); next = norm(out as stored), its int8 rows beside it
 //
 // Bound by memory: each row is read once into registers, 8 values a thread and step (16- or 32-byte accesses), normed there
-// and written once.  The squares are summed in 64 bits, whose order no result depends on (a sum in another order differs in
-// the 53rd bit; r is rounded to 24): int8 codes are then the same however a row is split over lanes, and equal those of
-// separate calls.  The 64-bit adds are two a value beside 4 or more bytes of memory traffic a value.
+// and written once.  The squares are summed in 64 bits and r is rounded to 24, so that another order of the sum, which moves it by
+// some 2^-53, moves r's last bit once in 10^8 rows.  The order goes by how a row is split over lanes (pick_split): for rows that
+// 16-byte accesses take, by their length alone, so that a token's result, int8 codes included, is the same in every batch, and up
+// to 4096 values in norms and joins alike (a wave's sum is that of 512 neighbouring values, the waves' are added in turn).  The
+// 64-bit adds are two a value beside 4 or more bytes of memory traffic a value.
 #include "xs_block.h"
 
 #include <type_traits>
@@ -228,16 +230,21 @@ namespace {
 template <int N>
 using Int = std::integral_constant<int, N>;
 
-// How a row is split: 8 values a thread, so that every row a call reads is asked for at once; from 4096 values on with many
-// rows 16, whose work-groups are smaller.  Measured (norm of fp32 rows to bf16, join with norms on both sides, us):
-// 2048 x 2048 7.1, 12.4 with 8 values a thread, 7.7, 15.0 with 16, 9.8, 20.6 with 32; 2048 x 4096 10.9, 24.9 / 11.3, 26.1 /
-// 12.5, 32.4; 1024 x 7168 11.2, 23.6 / 10.5, 24.8 / 12.6, 27.1; one row of 2048 2.5, 4.4 / 4.0, 4.6 / 4.3, 5.8.
+// How a row is split: 8 values a thread, so that every row a call reads is asked for at once; past 4096 values 16, whose
+// work-groups are smaller.  Measured (norm of fp32 rows to bf16, join with norms on both sides, us): 2048 x 2048 7.1, 12.4 with 8
+// values a thread, 7.7, 15.0 with 16, 9.8, 20.6 with 32; 2048 x 4096 10.9, 24.9 / 11.3, 26.1 / 12.5, 32.4; 1024 x 7168 11.2, 23.6 /
+// 10.5, 24.8 / 12.6, 27.1; one row of 2048 2.5, 4.4 / 4.0, 4.6 / 4.3, 5.8.
+// Rows of 16-byte accesses (VEC) are split the same in a call of any number of rows, so that their sums have one order; few rows
+// past 4096 values gain by it more than they lose (norm, join, join of 8 parts with 16 values a thread / 8: 7 x 7168 3.07, 4.54, 7.8 / 3.08, 4.67,
+// 8.2; 1 x 5120 2.79, 4.05, 6.8 / 2.75, 4.18, 6.4; 511 x 8192 7.07, 16.4, 38.8 / 6.78, 15.8, 39.7).  Others, one value an access,
+// take 8 values a thread below 512 rows (7 x 5121 3.39, 5.68, 8.2 / 3.70, 6.35, 10.4 with 16; 4096 x 5121 norm to bf16 27.9 / 22.0),
+// and so do int8 rows, whose maximum has no order.
 // TRIM, the waves that a row needs instead of the next power of two: 2 for norms and int8 rows (4096 x 2560, 5 waves / 8: norm to
 // int8 14.1 / 18.0, int8 rows 11.0 / 13.4; 4096 x 5120, 5 waves with 16 values a thread / 8: 22.2 / 28.0, 18.4 / 21.2); 1, up to
 // 4096 values, for a join of rows (bf16, 4096 x 2560 17.0 / 19.8, but 4096 x 5120 46.9 / 39.7); 0 for a join of parts, whose many
 // loads want the lanes (1024 x 2560 24.1 / 22.8, 1024 x 6144 52.5 / 49.0).
 template <int TRIM, typename F>
-hipError_t pick_split(int64_t rows, int n, F&& launch) {
+hipError_t pick_split(bool one_order, int64_t rows, int n, F&& launch) {
     if (n <= 512) return launch(Int<1>{}, Int<1>{});
     if (n <= 1024) return launch(Int<2>{}, Int<1>{});
     if constexpr (TRIM > 0) {
@@ -251,7 +258,7 @@ hipError_t pick_split(int64_t rows, int n, F&& launch) {
     }
     if (n <= 4096) return launch(Int<8>{}, Int<1>{});
     if (n > 8192) return launch(Int<16>{}, Int<2>{});
-    if (rows < 512) return launch(Int<16>{}, Int<1>{});
+    if (!one_order && rows < 512) return launch(Int<16>{}, Int<1>{});
     if constexpr (TRIM > 1) {
         if (n <= 5120) return launch(Int<5>{}, Int<2>{});
         if (n <= 6144) return launch(Int<6>{}, Int<2>{});
@@ -269,7 +276,7 @@ dim3 row_block() {
 }
 
 hipError_t launch_norm(const NormArgs& a, bool vec, hipStream_t s) {
-    return pick_split<2>(a.n_tok, a.n, [&](auto nw, auto ch) {
+    return pick_split<2>(vec, a.n_tok, a.n, [&](auto nw, auto ch) {
         constexpr int NW = decltype(nw)::value, CH = decltype(ch)::value;
         if (vec)
             hipLaunchKernelGGL((block_norm_kernel<NW, CH, true>), row_grid<NW>(a.n_tok), row_block<NW>(), 0, s, a);
@@ -280,7 +287,7 @@ hipError_t launch_norm(const NormArgs& a, bool vec, hipStream_t s) {
 }
 template <bool PARTS>
 hipError_t launch_join(const JoinArgs& a, bool vec, hipStream_t s) {
-    return pick_split<PARTS ? 0 : 1>(a.n_tok, a.n, [&](auto nw, auto ch) {
+    return pick_split<PARTS ? 0 : 1>(vec, a.n_tok, a.n, [&](auto nw, auto ch) {
         constexpr int NW = decltype(nw)::value, CH = decltype(ch)::value;
         if (vec)
             hipLaunchKernelGGL((block_join_kernel<NW, CH, true, PARTS>), row_grid<NW>(a.n_tok), row_block<NW>(), 0, s, a);
@@ -298,7 +305,7 @@ hipError_t launch_quantize(const QuantArgs& a, bool vec, hipStream_t s) {
             hipLaunchKernelGGL((w8a8_quantize_kernel<NW, CH, false>), row_grid<NW>(a.rows), row_block<NW>(), 0, s, a);
         return hipGetLastError();
     };
-    if (a.n <= 16384) return pick_split<2>(a.rows, a.n, go);
+    if (a.n <= 16384) return pick_split<2>(false, a.rows, a.n, go);
     if (a.n <= 32768) return go(Int<16>{}, Int<4>{});
     return go(Int<16>{}, Int<8>{});
 }
