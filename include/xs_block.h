@@ -73,7 +73,9 @@ int xs_block_join(const xs_block_join_cfg_t* J, const void* y, int y_type, int64
 
 /* The join of an MoE layer's parts: a token's block output is the weighted sum of its k rows of `parts` (routing order,
  * n_embd floats each) in rank order, + its row of `shared` once (times 1 / (1 + exp(-shared_gate[t])) where given, taken
- * as the token gate above) - xs_native_moe_combine_multi's sum, whose order and roundings it keeps.  k in 1 .. 15. */
+ * as the token gate above).  Order and roundings are xs_native_moe_combine_multi's, whose bits the sum has without
+ * shared_gate; that entry point takes the gate's sigmoid in fp32, four roundings where this one has one, so that a gated
+ * shared row's values may differ by 7 * 2^-24 of themselves before they are added.  k in 1 .. 15. */
 int xs_moe_combine_join(const xs_block_join_cfg_t* J, const float* parts, const float* weights, int64_t k,
                         const float* shared, const float* shared_gate, const void* residual, void* out, int r_type,
                         int64_t ldr, void* next, int next_type, int64_t ld_next, int8_t* q, int64_t ldq,

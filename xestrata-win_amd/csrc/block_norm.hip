@@ -1,7 +1,8 @@
 // xestrata-win_amd/csrc/block_norm.hip - the norm before a block and the join after one (include/xs_block.h).
 //
 //   norm   y = fl(fl(x r) w), r = fl(1 / sqrt(sum x^2 / n + eps)), the sum and the root in 64 bits
-//   join   b = the block's output (or the weighted parts, summed as combine.hip does); b = norm(b); b = fl(b g);
+//   join   b = the block's output (or the weighted parts, summed as combine.hip does but for a shared gate's
+//          sigmoid, which is taken in 64 bits here); b = norm(b); b = fl(b g);
 //          out = fl(fl(rs residual) + fl(bs b)); next = norm(out as stored), its int8 rows beside it
 //
 // Bound by memory: each row is read once into registers, 8 values a thread and step (16- or 32-byte accesses), normed there
