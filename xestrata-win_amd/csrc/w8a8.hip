@@ -316,6 +316,7 @@ __global__ __launch_bounds__(64 * WM * WN) void w8a8_tile_kernel(const W8Args a,
         for (int i = 0; i < FM; ++i)
             acc[h * JH + j][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wj[j], x[kk][i], acc[h * JH + j][i], 0, 0, 0);
     };
+    // (tests/test_w8a8_schedule.py compiles the lines from here to the sums, and the ring's loop, for the host)
     // asked for in the order in which they are waited for: x 0, w 0, ... x S - 1, w S - 1, w S
 #pragma unroll
     for (int s = 0; s <= S; ++s)
