@@ -120,3 +120,16 @@ def test_one_row_of_a_wider_buffers_weights(handed):
         assert handed == [w.data_ptr(), 3]
     with pytest.raises(xsmoe.XsError, match="6 values apart"):
         xsmoe.moe_combine_join(torch.ones(6, N), buffer[:2, :3], torch.ones(2, N), cfg)
+
+
+def test_one_tensor_in_two_places(handed):
+    """Each place asks for its own size, whichever tensor stands there."""
+    g = torch.ones(T)
+    for v in (dict(gate=g, gate_kind="token", next_w=g), dict(gate=g, gate_kind="token", norm=True, norm_w=g)):
+        with pytest.raises(xsmoe.XsError, match="_w is not 64"):
+            join(xsmoe.block_join_cfg(**v))
+    rows = torch.ones(T, N)
+    with pytest.raises(xsmoe.XsError, match="next_w is not 64"):
+        join(xsmoe.block_join_cfg(gate=rows, gate_kind="value", next_w=rows))
+    w = torch.ones(N)
+    join(xsmoe.block_join_cfg(gate=w, gate_kind="channel", next_w=w, norm=True, norm_w=w))

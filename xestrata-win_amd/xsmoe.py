@@ -791,34 +791,36 @@ def block_join_cfg(norm=False, norm_w=None, norm_eps=1e-6, gate=None, gate_kind=
     if norm_w is not None and not norm:
         raise _bad(f"{what}: norm weights without the norm")
     ld = _rows(what, "gate", gate, types=_F32_ONLY)[2] if gate_kind == "value" else 0
-    cfg = BlockJoinCfg(int(norm), _p(norm_w), norm_eps, GATE_KIND[gate_kind], _p(gate), ld, branch_scale,
-                       residual_scale, _p(next_w), next_eps)
-    cfg._keep = (norm_w, gate, next_w)
-    # (tokens, row length, device) that its tensors are for, None: any; -1 where they disagree: no call fits
+    # the tokens, row length and device that its tensors are for (None: any; -1 where they disagree: no call fits), and what each
+    # tensor was then
     T = n = dev = None
-    plain = True
-    for t, rows, size in ((norm_w, None, -2), (next_w, None, -2), (gate, *_GATE_FOR[gate_kind])):
+    plain, at, seen = True, [], []
+    for t, role in ((norm_w, "channel"), (gate, gate_kind), (next_w, "channel")):
         if t is None:
+            at.append(None)
             continue
-        at, many = t.get_device(), t.numel()
-        dev = at if dev is None or dev == at else -1
-        if size == -2:      # a vector of the row's length
-            n = many if n is None or n == many else -1
-        elif size == -3:    # rows of it
-            n = t.shape[1] if n is None or n == t.shape[1] else -1
-        if rows is not None:
-            T = many if size is None else t.shape[0]
-        plain = plain and t.dtype is torch.float32 and (size == -3 or t.is_contiguous()) and (t.data_ptr() != 0 or many == 0)
-    cfg._for, cfg._plain = (T, n, dev), plain
-    cfg._seen = [(t, t.data_ptr(), t.dtype, t.shape, t.stride()) for t in cfg._keep if t is not None]
+        p, many, kind, here = t.data_ptr(), t.numel(), t.dtype, t.get_device()
+        at.append(p)
+        dev = here if dev is None or dev == here else -1
+        plain = plain and kind is torch.float32 and (p != 0 or many == 0) and (role == "value" or t.is_contiguous())
+        seen.append((t, p, many, kind, (t.shape, t.stride()) if role == "value" else None))
+        if role == "token":
+            T = many
+            continue
+        if role == "value":
+            T, many = t.shape
+        n = many if n is None or n == many else -1
+    cfg = BlockJoinCfg(int(norm), at[0], norm_eps, GATE_KIND[gate_kind], at[1], ld, branch_scale, residual_scale, at[2], next_eps)
+    cfg._keep, cfg._for, cfg._plain, cfg._seen = (norm_w, gate, next_w), (T, n, dev), plain, seen
     return cfg
 
 
 def _as_it_is(cfg):
     """The configuration, made again (for this call) where one of its tensors has since been given other memory, another size,
     layout or type."""
-    for t, at, kind, shape, stride in cfg._seen:
-        if t.data_ptr() != at or t.dtype is not kind or t.shape != shape or t.stride() != stride:
+    for t, at, many, kind, layout in cfg._seen:
+        if t.data_ptr() != at or t.numel() != many or t.dtype is not kind or \
+                (not t.is_contiguous() if layout is None else (t.shape, t.stride()) != layout):
             norm_w, gate, next_w = cfg._keep
             return block_join_cfg(cfg.norm == 1, norm_w, cfg.norm_eps, gate, _GATE_NAME[cfg.gate_kind], cfg.branch_scale,
                                   cfg.residual_scale, next_w, cfg.next_eps)
@@ -826,8 +828,6 @@ def _as_it_is(cfg):
 
 
 _F32_ONLY = {torch.float32: 0}
-# of each gate kind: whether its rows are the tokens, and its length (None: says nothing; -2, -3 as in block_join_cfg)
-_GATE_FOR = {"none": (None, None), "token": (True, None), "channel": (None, -2), "value": (True, -3)}
 
 
 def _join(what, fn, head, x, residual, cfg, T, n, out, next_type, next, quant, q, scale, stream):
