@@ -811,19 +811,7 @@ def block_join_cfg(norm=False, norm_w=None, norm_eps=1e-6, gate=None, gate_kind=
             T, many = t.shape
         n = many if n is None or n == many else -1
     cfg = BlockJoinCfg(int(norm), at[0], norm_eps, GATE_KIND[gate_kind], at[1], ld, branch_scale, residual_scale, at[2], next_eps)
-    cfg._keep, cfg._for, cfg._plain, cfg._seen = (norm_w, gate, next_w), (T, n, dev), plain, seen
-    return cfg
-
-
-def _as_it_is(cfg):
-    """The configuration, made again (for this call) where one of its tensors has since been given other memory, another size,
-    layout or type."""
-    for t, at, many, kind, layout in cfg._seen:
-        if t.data_ptr() != at or t.numel() != many or t.dtype is not kind or \
-                (not t.is_contiguous() if layout is None else (t.shape, t.stride()) != layout):
-            norm_w, gate, next_w = cfg._keep
-            return block_join_cfg(cfg.norm == 1, norm_w, cfg.norm_eps, gate, _GATE_NAME[cfg.gate_kind], cfg.branch_scale,
-                                  cfg.residual_scale, next_w, cfg.next_eps)
+    cfg._keep, cfg._for = (norm_w, gate, next_w), (T, n, dev, plain, seen)
     return cfg
 
 
@@ -833,9 +821,17 @@ _F32_ONLY = {torch.float32: 0}
 def _join(what, fn, head, x, residual, cfg, T, n, out, next_type, next, quant, q, scale, stream):
     """What block_join and moe_combine_join share: the configuration's and the outputs' checks, then the call."""
     dev = x.get_device()
-    cfg = _as_it_is(cfg)
-    rows, size, at = cfg._for
-    if not (cfg._plain and (rows is None or rows == T) and (size is None or size == n) and (at is None or at == dev)):
+    rows, size, at, plain, seen = cfg._for
+    for t, p, many, kind, layout in seen:
+        if t.data_ptr() != p or t.numel() != many or t.dtype is not kind or \
+                (not t.is_contiguous() if layout is None else (t.shape, t.stride()) != layout):
+            # it has been given other memory, another size, layout or type: the configuration is made again, for this call
+            norm_w, gate, next_w = cfg._keep
+            cfg = block_join_cfg(cfg.norm == 1, norm_w, cfg.norm_eps, gate, _GATE_NAME[cfg.gate_kind], cfg.branch_scale,
+                                 cfg.residual_scale, next_w, cfg.next_eps)
+            rows, size, at, plain, _ = cfg._for
+            break
+    if not (plain and (rows is None or rows == T) and (size is None or size == n) and (at is None or at == dev)):
         norm_w, gate, next_w = cfg._keep   # one of them does not fit: say which
         _vec(what, "norm_w", norm_w, n, dev)
         _vec(what, "next_w", next_w, n, dev)
