@@ -177,12 +177,16 @@ def prepare(case, seed):
             s.shared = _rows(g, T, H)
         if case["shared"] == "gated":
             s.shared_gate = torch.randn(T, generator=g, device=DEV)
-    if own:
-        xm = _library()
-        s.join = xm.block_join_cfg(norm=case["norm"], norm_w=s.norm_w, norm_eps=EPS, gate=s.gate, gate_kind=case["gate"],
-                                   branch_scale=s.branch_scale, residual_scale=s.residual_scale, next_w=s.next_w,
-                                   next_eps=EPS)
+    # a token's or a value's gate is computed for the call, its configuration made with it; what holds only weights is kept
+    s.join = _join_cfg(s) if own and case["gate"] in ("none", "channel") else None
     return s
+
+
+def _join_cfg(s):
+    c = s.case
+    return _library().block_join_cfg(norm=c["norm"], norm_w=s.norm_w, norm_eps=EPS, gate=s.gate, gate_kind=c["gate"],
+                                     branch_scale=s.branch_scale, residual_scale=s.residual_scale, next_w=s.next_w,
+                                     next_eps=EPS)
 
 
 def _library():
@@ -214,10 +218,11 @@ def _run_own(s):
         return _out(y=y, values=_values(q, scale), scale=scale)
     if c["do"] in ("join", "combine"):
         want = dict(next_type=FLOAT.get(c["next"]), quant=c["quant"])
+        cfg = s.join or _join_cfg(s)
         if c["do"] == "join":
-            out, nxt, q, scale = xm.block_join(s.y, s.residual, s.join, **want)
+            out, nxt, q, scale = xm.block_join(s.y, s.residual, cfg, **want)
         else:
-            out, nxt, q, scale = xm.moe_combine_join(s.parts, s.weights, s.residual, s.join, shared=s.shared,
+            out, nxt, q, scale = xm.moe_combine_join(s.parts, s.weights, s.residual, cfg, shared=s.shared,
                                                      shared_gate=s.shared_gate, **want)
         return _out(out=out, next=nxt, values=_values(q, scale), scale=scale)
     if c["do"] == "product":
