@@ -7,8 +7,8 @@
  *
  * Conventions are include/xs_moe.h's: device memory of the caller, nothing allocated, no state between calls (calls on
  * different streams share nothing), return codes and xs_last_error(); a NULL stream is HIP's default stream and the call
- * then synchronises.  Zero or fewer tokens: nothing is done; norms, joins and quantizations take up to 2^21.  Rows are n values long and ld values apart (ld >= n);
- * what lies between is neither read as data nor written.  Every pointer is aligned to its values' size; outputs overlap no
+ * then synchronises.  Zero or fewer tokens: nothing is done; norms, joins and quantizations take up to 2^21.  Rows are n
+ * values long and ld values apart (ld >= n); what lies between is neither read as data nor written.  Every pointer is aligned to its values' size; outputs overlap no
  * input and no other output, except where an entry says so; columns of one buffer (rows of one stride between each
  * other's) are apart.
  *
@@ -16,7 +16,8 @@
  * rounded on its own, and rounded once more (to nearest even) where they are stored in 16 bits.
  *
  * int8 rows: codes q and a float scale s a row; the row's values are q s.  A row of values v is quantized as
- *   s = max(max |v| fl(1 / 127), 2^-126) (one product, as xs_quantize_q8_1_rows takes its scale),
+ *   s = max(max |v| fl(1 / 127), 2^-126) (one product, as xs_quantize_q8_1_rows takes its scale: within 0.57 steps of
+ *       max |v| / 127),
  *   q = the integer nearest the exact v / s (halves to even);
  * a row that holds a NaN or an infinity gets s = NaN and q = 0, so everything computed from it is NaN.
  */
@@ -35,7 +36,8 @@ extern "C" {
 #define XS_BF16 30
 
 /* The norm before a block: y[t, c] = (x[t, c] r) w[c], r = 1 / sqrt(mean of x[t, .]^2 + eps) (the mean and the root in 64
- * bits, r rounded once).  w NULL: no weights.  y (y_type, ldy) and the int8 rows of the fp32 y (q, ldq bytes apart, and
+ * bits, r rounded once; rows that 16-byte accesses take give the same bits in a call of any number of rows, other rows may
+ * differ in r's last bit).  w NULL: no weights.  y (y_type, ldy) and the int8 rows of the fp32 y (q, ldq bytes apart, and
  * q_scale [n_tok]) are written where given; one of them has to be.  y may be x itself (the same type and ld).
  * n_embd 1 .. 16384; eps finite, not negative. */
 int xs_block_norm(const void* x, int x_type, int64_t ldx, const float* w, float eps, void* y, int y_type, int64_t ldy,

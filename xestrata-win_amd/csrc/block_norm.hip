@@ -202,7 +202,8 @@ __global__ __launch_bounds__(NW == 1 ? 256 : 64 * NW) void block_join_kernel(con
     }
 }
 
-// rows of any length up to 65536 to int8 rows
+// Rows of any length up to 65536 to int8 rows.  Bound by memory; past 32768 values a row's 64 values a thread take all of 128
+// registers and spill 2 to 4 (4096 x 65536 fp32 302 us, 4.4 TB/s; bf16 219 us; 4096 x 7168 26.2 us, 5.6 TB/s).
 struct QuantArgs {
     const void* x;
     int8_t* q;
@@ -236,10 +237,10 @@ using Int = std::integral_constant<int, N>;
 // values a thread, 7.7, 15.0 with 16, 9.8, 20.6 with 32; 2048 x 4096 10.9, 24.9 / 11.3, 26.1 / 12.5, 32.4; 1024 x 7168 11.2, 23.6 /
 // 10.5, 24.8 / 12.6, 27.1; one row of 2048 2.5, 4.4 / 4.0, 4.6 / 4.3, 5.8.
 // Rows of 16-byte accesses (VEC) are split the same in a call of any number of rows, so that their sums have one order; few rows
-// past 4096 values gain by it more than they lose (norm, join, join of 8 parts with 16 values a thread / 8: 7 x 7168 3.07, 4.54, 7.8 / 3.08, 4.67,
-// 8.2; 1 x 5120 2.79, 4.05, 6.8 / 2.75, 4.18, 6.4; 511 x 8192 7.07, 16.4, 38.8 / 6.78, 15.8, 39.7).  Others, one value an access,
-// take 8 values a thread below 512 rows (7 x 5121 3.39, 5.68, 8.2 / 3.70, 6.35, 10.4 with 16; 4096 x 5121 norm to bf16 27.9 / 22.0),
-// and so do int8 rows, whose maximum has no order.
+// past 4096 values gain by it more than they lose (norm, join, join of 8 parts with 16 values a thread / 8: 7 x 7168 3.07, 4.54,
+// 7.8 / 3.08, 4.67, 8.2; 1 x 5120 2.79, 4.05, 6.8 / 2.75, 4.18, 6.4; 511 x 8192 7.07, 16.4, 38.8 / 6.78, 15.8, 39.7).  Others, one
+// value an access, take 8 values a thread below 512 rows (7 x 5121 3.39, 5.68, 8.2 / 3.70, 6.35, 10.4 with 16; 4096 x 5121 norm to
+// bf16 27.9 / 22.0), and so do int8 rows, whose maximum has no order.
 // TRIM, the waves that a row needs instead of the next power of two: 2 for norms and int8 rows (4096 x 2560, 5 waves / 8: norm to
 // int8 14.1 / 18.0, int8 rows 11.0 / 13.4; 4096 x 5120, 5 waves with 16 values a thread / 8: 22.2 / 28.0, 18.4 / 21.2); 1, up to
 // 4096 values, for a join of rows (bf16, 4096 x 2560 17.0 / 19.8, but 4096 x 5120 46.9 / 39.7); 0 for a join of parts, whose many

@@ -8,8 +8,8 @@ namespace xs {
 
 // The kernels' shapes and what a work-group of each costs, in ns: a step of 128 bytes of k `alone`, with up to as many on the
 // chip as CUs, `each` for every one of a CU where several share it (0: they do not, and go in rounds), and what is `fixed` beside
-// the steps, the start and the outputs.  Fitted to measurements at 48 to 8192 inputs; what bounds them all is what the L2s give
-// the CUs, so that a step goes by the rows that a shape reads (tokens + weights).
+// the steps, the start and the outputs.  Fitted to measurements at 48 to 8192 inputs; a step goes by the rows that a shape reads
+// (tokens + weights).
 struct Shape {
     int tokens, rows;   // of a work-group; GATED: rows / 2 outputs
     int alone, each, fixed;
@@ -28,7 +28,8 @@ constexpr Shape kShapes[] = {
 constexpr int kShapeCount = sizeof kShapes / sizeof kShapes[0];
 
 // The shape that costs a call least: over 240 calls of 18 to 4096 tokens, 128 to 8192 outputs and 48 to 8192 inputs it takes
-// 1.016 times the best shape's time in the mean, 1.23 at worst (a 5 us call).  E.g. (tokens x outputs x inputs, us: it / another):
+// 1.016 times the best shape's time in the mean, 1.23 at worst (a 5 us call); over 69 of 24 to 4096 tokens, 512 to 4096 outputs and
+// 12288 to 65536 inputs 1.008, 1.15 at worst (a gated 64 x 512 x 65536: 32 x 32 43 us, 16 x 16 38).  E.g. (tokens x outputs x inputs, us: it / another):
 // 24 x 2048 x 4096: 16 x 16 5.0 / 32 x 32 7.0; 37 x 2050 x 7168: 32 x 32 8.4 / 64 x 32 10.3; 64 x 8192 x 4096: 64 x 32 12.2 / 32 x
 // 32 12.8; 200 x 4096 x 4096: 64 x 64 ring 11.1 / 64 x 32 13.8; 300 x 2594 x 4208: 64 x 64 tile 14.8 / ring 17.0; 512 x 4096 x
 // 4096: 64 x 128 17.3 / 64 x 64 18.0; 4096 x 2048 x 256: 128 x 128 9.6 / 128 x 256 10.1; 1024 x 4096 x 4096: 128 x 128 24 / 64 x 64

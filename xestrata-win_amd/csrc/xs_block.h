@@ -18,7 +18,10 @@ __host__ __device__ constexpr int float_bytes(int t) { return t == XS_F32 ? 4 : 
 
 // ---------------------------------------------------------------- the int8 rule
 // The scale of a row whose largest |v| has the bits `amax`: never under the smallest normal number, so that 1 / s is finite
-// and a code's product with it exact; NaN where the row holds an infinity or a NaN (their bits are the largest of all).
+// and a code's product with it exact; NaN where the row holds an infinity or a NaN (their bits are the largest of all).  The
+// product with the rounded 1 / 127 (0.06 steps off at most) is within 0.57 steps of the quotient, where a division is within 0.5
+// (4.7% of the scales differ by one step); it is how the q8_1 rows take theirs.  What the codes stand for is as near either way:
+// they are the nearest to v / s for the s that is stored, and the largest |v| / s is within 127 (1 + 2^-23), which is 127.
 __device__ __forceinline__ float int8_scale(uint32_t amax) {
     if (amax >= 0x7F800000u) return u2f(0x7FC00000u);
     return fmaxf(u2f(amax) * (1.0f / 127.0f), 1.17549435e-38f);

@@ -646,8 +646,8 @@ class MoeLayer:
 # ------------------------------------------------------------------------------------------------ around the layer
 # include/xs_block.h: the norm before a block, the join after one, int8 products.  Rows are 2-D tensors whose last
 # dimension is contiguous (any row stride); int8 rows are (q, scale): q [rows, n] int8 with rows of a whole number of 16
-# bytes (a view, as w8a8_quantize makes them), scale [rows] fp32.  Tensors that are missing, on the host, on different
-# devices, of another type or shape raise XsError before anything is launched.
+# bytes (a view, as w8a8_quantize makes them), scale [rows] fp32.  With `stream`, new results are that stream's memory.  Tensors
+# that are missing, on the host, on different devices, of another type or shape raise XsError before anything is launched.
 
 FLOAT_TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 INT8_TYPE = {torch.int8: 24}
@@ -858,7 +858,9 @@ def _join(what, fn, head, x, residual, cfg, T, n, out, next_type, next, quant, q
 
 def block_join(y, residual, cfg, out=None, next_type=None, quant=False, next=None, q=None, scale=None, stream=None):
     """A block's rows y [T, n] joined to the residual (cfg: block_join_cfg) -> (out, next, q, scale): the new residual and,
-    with next_type (or next) and / or quant (or q and scale), the next block's norm of it as rows and as int8 rows."""
+    with next_type (or next) and / or quant (or q and scale), the next block's norm of it as rows and as int8 rows.
+    out (it may be the residual) has the residual's row stride; a new one of a residual that is columns of a wider buffer
+    takes as much memory as those rows span."""
     T, n, ldy, yt = _rows("block_join", "y", y)
     return _join("block_join", lib().xs_block_join, (y.data_ptr(), yt, ldy), y, residual, cfg, T, n, out, next_type, next,
                  quant, q, scale, stream)
