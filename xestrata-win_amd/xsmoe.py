@@ -646,8 +646,10 @@ class MoeLayer:
 # ------------------------------------------------------------------------------------------------ around the layer
 # include/xs_block.h: the norm before a block, the join after one, int8 products.  Rows are 2-D tensors whose last
 # dimension is contiguous (any row stride); int8 rows are (q, scale): q [rows, n] int8 with rows of a whole number of 16
-# bytes (a view, as w8a8_quantize makes them), scale [rows] fp32.  With `stream`, new results are that stream's memory.  Tensors
-# that are missing, on the host, on different devices, of another type or shape raise XsError before anything is launched.
+# bytes (a view, as w8a8_quantize makes them), scale [rows] fp32.  With `stream`, new results are that stream's memory;
+# inputs made on another stream are the caller's to order and to keep until the call has run, as for torch's own operations.
+# Tensors that are missing, on the host, on different devices, of another type or shape raise XsError before anything is
+# launched.
 
 FLOAT_TYPE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 INT8_TYPE = {torch.int8: 24}
